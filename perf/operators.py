@@ -7,10 +7,6 @@ autograd for ``sageattn_train``; forward, or forward and gradients, for ``rotary
 
 ``own`` false computes the same outputs in plain elementary operations.
 """
-import functools
-import os
-import sys
-
 import torch
 
 own = False
@@ -18,9 +14,10 @@ own = False
 DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
 
 
-@functools.lru_cache(maxsize=None)
 def _own():
-    """The package, imported once."""
+    import os
+    import sys
+
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sageattention-rdna3_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)

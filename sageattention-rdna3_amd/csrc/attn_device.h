@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <cfloat>
 
 #include "sage_common.h"
 
@@ -104,15 +105,23 @@ __device__ __forceinline__ float row_lse(float m, float l) {
   return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
-// The reference max that a tile max moves a row to.  A score minus it is one
-// fma of the unrounded score, so it may come out above 0 by the rounding of the
-// max itself: nothing below 2^24, but up to 2^100 where keys are masked with
-// the lowest value of a type, and exp2 of that is infinite.  From 2^24 on the
-// max is rounded up by a step, which keeps every difference at or below 0.
-// (-inf gives NaN, which the max with the old reference drops.)
-__device__ __forceinline__ float ref_max(float mx) {
-  const float a = __builtin_fabsf(mx);
-  return a < 0x1p24f ? mx : __builtin_fmaf(a, 0x1p-23f, mx);
+// A score minus the reference max is one fma of the unrounded score, so the
+// largest key's may miss 0 by the rounding of the max itself: at most a half
+// below 2^24, but up to 2^100 where keys are masked with the lowest value of a
+// type, either way (P infinite, or 0 for every key).  Rows with a reference max
+// from 2^24 on round the score like the max instead (huge_score), which makes
+// that difference 0 and every other one negative; the score's own fp32 sum is
+// off by as much.  Such a row's max moves with every tile (a step of it is more
+// than the lazy threshold), so it is never behind a score.  (-FLT_MAX is a row
+// without a live key so far.)
+__device__ __forceinline__ bool huge_ref(float m) {
+  const float a = __builtin_fabsf(m);
+  return a >= 0x1p24f && a < FLT_MAX;
+}
+__device__ __forceinline__ float huge_score(float x, float sc, float m) {
+#pragma clang fp contract(off)
+  const float s = x * sc;
+  return huge_ref(m) ? s - m : __builtin_fmaf(x, sc, -m);
 }
 
 // Uniform 64-bit pointer (the compiler cannot always prove it).

@@ -229,8 +229,10 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_attn_kernel(FewParams p) {
 
   float16_t_ o[RT][C::kDB];
   float m_run[RT], l_run[RT];
+  bool huge[RT];  // a row's reference max is 2^24 or more (see huge_ref)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
+    huge[rt] = false;
     m_run[rt] = -FLT_MAX;  // see the softmax: finite, so that a tile of -inf scores gives p = 0
     l_run[rt] = 0.0f;
 #pragma unroll
@@ -374,12 +376,13 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_attn_kernel(FewParams p) {
       // the lowest finite value: a row whose scores are all -inf so far (keys
       // masked through K) has p = exp2(-inf) = 0 against it, where -inf would
       // give exp2(-inf + inf), and the first live score moves it
-      if (__builtin_amdgcn_ballot_w64(mx > m_run[rt] + kFewRescale) != 0) {
+      if (huge[rt] || __builtin_amdgcn_ballot_w64(mx > m_run[rt] + kFewRescale) != 0) {
         asm volatile("");  // a real branch
-        float m_new = __builtin_fmaxf(m_run[rt], ref_max(mx));
+        float m_new = __builtin_fmaxf(m_run[rt], mx);
         if constexpr (I8) m_new = __builtin_ceilf(m_new);
         const float alpha = fast_exp2(m_run[rt] - m_new);
         m_run[rt] = m_new;
+        huge[rt] = __builtin_amdgcn_ballot_w64(huge_ref(m_new)) != 0;
         l_run[rt] *= alpha;
 #pragma unroll
         for (int db = 0; db < C::kDB; ++db) {
@@ -388,8 +391,14 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_attn_kernel(FewParams p) {
         }
       }
       // score - max in one rounding: scores may be far larger than their differences
+      if (huge[rt]) {
+        asm volatile("");  // a real branch
 #pragma unroll
-      for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc[r >> 3], -m_run[rt]);
+        for (int r = 0; r < 16; ++r) y[r] = huge_score(y[r], sc[r >> 3], m_run[rt]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc[r >> 3], -m_run[rt]);
+      }
       mask();
       float sum[2] = {0.0f, 0.0f};
       uint32_t pw[8];

@@ -164,7 +164,8 @@ int sage_attn_i8_fwd(const int8_t* q_i8, const int8_t* k_i8, const void* value_t
  * after dequantisation (the log2-domain score times ln 2), -inf for a row with
  * no live key (output 0), NaN where the output is NaN.  The reference's return_lse returns a zero placeholder instead
  * (sageattention/core.py:203-211); this is the value that placeholder stands
- * for, usable to merge partial attentions over split key ranges.
+ * for, usable to merge partial attentions over split key ranges (not where
+ * each range's K had its own mean subtracted: s_ij is then that of k_j - mean).
  */
 int sage_attn_i8_fwd_lse(const int8_t* q_i8, const int8_t* k_i8, const void* value_t, void* out,
                          float* lse, const float* q_scale, const float* k_scale, int out_dtype,
@@ -387,7 +388,8 @@ int sage_attn_few_fwd(int quantized, const void* query, const void* key, const v
  * off by about 2^-22 |lse| of themselves.
  * dq, or dk and dv together, may be NULL (not computed).  K and V have to be
  * finite also where a key is masked by its scores (0 times infinity).  dq, dk
- * and dv must not overlap an input.
+ * and dv must not overlap an input.  After a forward call on K minus its mean
+ * (smooth_k) key has to be K minus that mean: lse is that of those scores.
  * strides: (batch, head, token) strides in elements of dout, query, key,
  * value, out, dq, dk, dv, in this order (24 values); rows must not overlap.
  * workspace: sage_attn_bwd_workspace_bytes, 16-byte aligned, no

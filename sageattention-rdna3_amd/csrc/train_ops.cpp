@@ -282,9 +282,23 @@ py::object sageattn_train(at::Tensor q, at::Tensor k, at::Tensor v, const py::ob
   return py::cast(r[0]);
 }
 
+// k minus its mean over the tokens, as the INT8 path's smooth_k takes it (and rounds it, more coarsely than here).
+at::Tensor smoothed(const at::Tensor& key, int64_t layout) {
+  const at::Tensor k = rows_ready(key, layout);
+  const Dims d = bhnd(k, layout);
+  if (d.b == 0 || d.n == 0) return k;
+  const int64_t bytes = sage_k_mean_workspace_bytes(d.b, d.h, d.n, d.d);
+  check_std("sage_k_mean_workspace_bytes", bytes);
+  at::Tensor mean = at::empty({d.b, d.h, d.d}, k.options());
+  at::Tensor ws = at::empty({(std::max<int64_t>(bytes, 4) + 3) / 4}, k.options().dtype(at::kFloat));
+  check_std("sage_k_mean", sage_k_mean(k.data_ptr(), mean.data_ptr(), ws.data_ptr(), dtype_code(k), d.b, d.h, d.n, d.d,
+                                       d.sb, d.sh, d.sn, current_stream(k)));
+  return k - mean.unsqueeze(layout == 1 ? 2 : 1);
+}
+
 py::object sageattn_backward(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
                              const py::object& tensor_layout, bool is_causal, std::optional<double> sm_scale,
-                             const std::optional<at::Tensor>& dlse) {
+                             const std::optional<at::Tensor>& dlse, bool smooth) {
   const int64_t layout = layout_code(tensor_layout);
   check_qkv(q, k, v, layout);
   for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>("dout", &dout), {"out", &out}})
@@ -297,7 +311,10 @@ py::object sageattn_backward(at::Tensor dout, at::Tensor q, at::Tensor k, at::Te
     require_value(t == nullptr || (t->sizes() == at::IntArrayRef(rows) && t->scalar_type() == at::kFloat && t->device() == q.device()),
                   std::string(name) + " must be [" + std::to_string(d.b) + ", " + std::to_string(d.h) + ", " +
                       std::to_string(d.n) + "] fp32 on the device of q");
+  require_value(!smooth || dlse == std::nullopt, "dlse is not taken with smooth_k=True");
   const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(q.device());
+  if (smooth) k = smoothed(k, layout);
   AttnGrads g = attn_bwd(dout, q, k, v, out, lse, dlse ? *dlse : at::Tensor(), layout, is_causal, scale_or_default(sm_scale, q), true, true);
   return py::make_tuple(g.dq, g.dk, g.dv);
 }

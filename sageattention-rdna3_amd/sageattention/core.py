@@ -87,7 +87,8 @@ def sageattn(
     q: [B,Hq,Sq,D] (HND) or [B,Sq,Hq,D] (NHD); k, v with Hkv heads (Hq % Hkv == 0).
     Returns o with q's shape, layout and dtype (and, when ``return_lse``, the
     rows' log-sum-exp [B,Hq,Sq] fp32: ln sum_j exp(sm_scale * q_i.k_j) after
-    quantisation, -inf for a row with no key, NaN for a NaN row; the reference returns zeros).
+    quantisation, -inf for a row with no key, NaN for a NaN row; the reference returns zeros.
+    With ``smooth_k`` on the INT8 path k_j is the key minus the mean of the keys).
     ``bm_sel`` (the reference's experimental direct-kernel tile override) is
     accepted and ignored; other unknown kwargs are ignored too.
     """

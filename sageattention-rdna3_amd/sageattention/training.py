@@ -57,6 +57,7 @@ def sageattn_backward(
     is_causal: bool = False,
     sm_scale: Optional[float] = None,
     dlse: Optional[torch.Tensor] = None,
+    smooth_k: bool = False,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv) of an attention call from its inputs, its output and its log-sum-exp, for
     programs that keep those themselves: ``out, lse = sageattn(..., return_lse=True)`` (of either
@@ -64,8 +65,18 @@ def sageattn_backward(
     over key ranges merged by their LSEs (pass the merged output and LSE with each range's k, v).
 
     dout and out have q's shape, layout and dtype; lse and dlse (the LSE's gradient, optional) are
-    [B,Hq,Sq] fp32."""
-    return core._host().sageattn_backward(dout, q, k, v, out, lse, tensor_layout, is_causal, sm_scale, dlse)
+    [B,Hq,Sq] fp32.
+
+    ``smooth_k`` has to be what the forward call was given: with it the INT8 path attends over k minus
+    its mean over the tokens, and its LSE is that of those scores.  (The output and the gradients do
+    not depend on the shift; short calls, which take the direct kernel, have none.)  The LSEs of
+    smoothed calls over several key ranges cannot be merged, each having its own shift, and dlse is
+    refused with it."""
+    if smooth_k and getattr(q, "ndim", 0) == getattr(k, "ndim", 0) == 4 and tensor_layout in ("HND", "NHD"):
+        seq = 2 if tensor_layout == "HND" else 1
+        smooth_k = not core.use_direct_path(q.shape[3], q.shape[seq], k.shape[seq], bool(is_causal), tensor_layout)
+    return core._host().sageattn_backward(dout, q, k, v, out, lse, tensor_layout, is_causal, sm_scale, dlse,
+                                          bool(smooth_k))
 
 
 def rotary_axes(

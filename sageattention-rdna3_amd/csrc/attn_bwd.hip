@@ -28,9 +28,11 @@
 // Roundings: scores, probabilities, dP, delta and all sums are fp32; P and dS
 // are rounded once to the input type as operands of the last two products.
 // fp16 has too few exponents for that: P is scaled by 2^14 (as small as 1/n for
-// n keys), and dS by a power of two from a bound on |dP - delta| of the kv head
-// (from the largest row norms of dO and V), so neither overflows and only
-// values 2^-28 below the largest lose bits; both come off the fp32 sums.
+// n keys), and dS by a power of two from a bound on |dP - delta| of the kv head:
+// the largest row norms of dO and of the V at hand, and the largest |delta|,
+// which an output merged from other key ranges can make far larger than those.
+// So neither overflows and only values 2^-28 below the largest lose bits; both
+// come off the fp32 sums.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -66,7 +68,7 @@ struct ItemOrder {
 struct BwdParams {
   Rows q, k, v, dout, dq, dk, dv;  // dq null: no Q items; dk and dv null: no KV items
   const float* stat;  // [B*Hq][stat_tiles][2][32]: -L log2 e (-inf: P = 0; fp16: + kF16PScale), -delta
-  const float* omax;  // fp16: [B*Hq][omax_n][2]: largest row norm of dO, largest |dL|
+  const float* omax;  // fp16: [B*Hq][omax_n][2]: largest row norm of dO, largest |delta|, of rows with a live key
   const float* vmax;  // fp16: [B*Hkv][vmax_n]: largest row norm of V
   float* part;        // fp32 partial sums of split items
   int64_t q_part;     // where the Q pieces start, in tiles of kOwnRows x D
@@ -159,7 +161,7 @@ __device__ __forceinline__ int ds_exponent(const BwdParams& p, int bhk, char* sm
     vm = __builtin_fmaxf(vm, s[3 * w + 2]);
   }
   __syncthreads();
-  const float bound = 2.0f * om * vm + lm;  // of |dP - delta|
+  const float bound = om * vm + lm;  // of |dP - delta|
   int e = 0;
   if (bound > 0.0f && bound < INFINITY) e = 1 - static_cast<int>((__float_as_uint(bound) >> 23) & 255) + 126;
   return __builtin_amdgcn_readfirstlane(min(max(e, -100), 100));
@@ -516,9 +518,9 @@ __global__ __launch_bounds__(kBwdThreads, BwdCfg<D>::kWaves) void attn_bwd_kerne
 }
 
 // Row statistics: -L log2 e and -delta of kStatRows query rows a block (rows
-// past the last: P = 0), and for fp16 the largest row norms of dO and V that
-// bound dS (rows that are not finite left out: their own results are not
-// either).  HBM-bound: reads O and dO (fp16: and V) once.
+// past the last: P = 0), and for fp16 the largest row norms of dO and V and the
+// largest |delta|, which bound dS (rows that are not finite left out: their own
+// results are not either; and rows without a live key: they have no dS).  HBM-bound: reads O and dO (fp16: and V) once.
 //
 // O's rounding makes an error in delta that weighs like 1 / n in the dS of a row
 // of n keys (n = 1: dS is 0, and that error all that is left).  Rows of up to
@@ -640,23 +642,21 @@ __global__ __launch_bounds__(256) void attn_bwd_rows_kernel(PreParams p) {
       // what P lack of 1 may belong to keys elsewhere: below 2^-14 it weighs less than O's rounding in either type
       if (__builtin_fabsf(e.x - 1.0f) <= 0x1p-14f) dot = e.y;
     }
+    // a row without a live key: P = 0 everywhere, and its (arbitrary) delta must not meet it as NaN
+    const bool live = is_v || (row < n && !(wl[x] < kDeadLse));
     if (!is_v && c == 0) {
       const int tile = row / 32;
       float nl = -INFINITY, nd = 0.0f;
-      if (row < n) {
-        const float l = wl[x], dl = wd[x];
-        // a row without a live key: P = 0 everywhere, and its (arbitrary) delta must not meet it as NaN
-        if (!(l < kDeadLse)) {
-          nl = l * -1.4426950408889634f + (BF16 ? 0.0f : kF16PScale);
-          nd = dl - dot;
-        }
-        if (__builtin_fabsf(dl) < INFINITY) lmax = __builtin_fmaxf(lmax, __builtin_fabsf(dl));
+      if (live) {
+        nl = wl[x] * -1.4426950408889634f + (BF16 ? 0.0f : kF16PScale);
+        nd = wd[x] - dot;
+        if (__builtin_fabsf(nd) < INFINITY) lmax = __builtin_fmaxf(lmax, __builtin_fabsf(nd));
       }
       float* st = p.stat + (static_cast<int64_t>(bh) * p.stat_tiles + tile) * 64 + row % 32;
       st[0] = nl;
       st[32] = nd;
     }
-    if (sq < INFINITY) norm = __builtin_fmaxf(norm, sq);
+    if (live && sq < INFINITY) norm = __builtin_fmaxf(norm, sq);
   }
   if constexpr (!BF16) {
     norm = wave_max64(norm);

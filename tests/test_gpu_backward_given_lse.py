@@ -61,3 +61,49 @@ def test_smoothed_empty():
         lse = torch.zeros(b, 2, sq, device="cuda")
         got = sageattn_backward(dout, q, k, v, q, lse, smooth_k=True)
         assert [x.shape for x in got] == [q.shape, k.shape, v.shape] and not any(x.any() for x in got)
+
+
+def merged(q, k, v, dout, ranges, dtype, dlse=None, slack=0.0):
+    """The gradients of attention over all keys from calls over the ranges, each with the whole output and LSE: dk and dv
+    side by side, dq summed (each range's own rounded once more)."""
+    from sageattention import sageattn_backward, sageattn_train
+
+    out, lse = sageattn_train(q, k, v, return_lse=True)
+    want, bounds = reference(q, k, v, dout, "HND", False, dlse=dlse)
+    e = bounds(dtype)
+    parts = [sageattn_backward(dout, q, k[:, :, r], v[:, :, r], out, lse, dlse=dlse) for r in ranges]
+    for i, name in ((1, "dk"), (2, "dv")):
+        check(torch.cat([p[i] for p in parts], 2), want[name], e[name], "HND", name)
+    dq = [p[0].double() for p in parts]
+    check(sum(dq), want["dq"], e["dq"] + torch.finfo(dtype).eps / 2 * sum(x.abs() for x in dq), "HND", "dq")
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, F16), (128, BF16)])
+@pytest.mark.parametrize("dout_scale", [1.0, 64.0])
+@pytest.mark.parametrize("small", [0.0, 1e-3])
+@pytest.mark.parametrize("n", [64, 300])
+def test_merged_ranges_of_unlike_values(d, dtype, dout_scale, small, n):
+    """One range's V is far smaller than the other's, or zero (a padded block): delta is the merged output's, which that
+    range's V does not bound."""
+    q, k, v, dout = inputs(1, 2, 2, 150, 2 * n, d, dtype, "HND", seed=11, dout_scale=dout_scale)
+    v[:, :, n:] *= small
+    merged(q, k, v, dout, (slice(0, n), slice(n, 2 * n)), dtype)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_dead_rows_do_not_scale(d):
+    """fp16 scales dS by the largest row of a kv head: a row without a live key has no dS and does not count, however
+    large its gradients are."""
+    from sageattention import sageattn, sageattn_backward
+
+    q, k, v, dout = inputs(1, 2, 2, 100, 100, d, F16, "HND", dout_scale=1e-3)
+    out, lse = sageattn(q, k, v, return_lse=True)
+    dlse = torch.zeros_like(lse)
+    lse[:, :, ::7] = float("-inf")
+    dout[:, :, ::7] = 0
+    want = sageattn_backward(dout, q, k, v, out, lse, dlse=dlse)
+    dlse[:, :, ::7] = 1e30
+    out[:, :, ::7] = 6e4
+    dout[:, :, ::7] = 6e4
+    for x, y in zip(sageattn_backward(dout, q, k, v, out, lse, dlse=dlse), want):
+        assert torch.equal(x, y)

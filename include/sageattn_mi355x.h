@@ -390,6 +390,7 @@ int sage_attn_few_fwd(int quantized, const void* query, const void* key, const v
  * finite also where a key is masked by its scores (0 times infinity).  dq, dk
  * and dv must not overlap an input.  After a forward call on K minus its mean
  * (smooth_k) key has to be K minus that mean: lse is that of those scores.
+ * A probability above 1 (an lse of quantised scores) counts as 1.
  * strides: (batch, head, token) strides in elements of dout, query, key,
  * value, out, dq, dk, dv, in this order (24 values); rows must not overlap.
  * workspace: sage_attn_bwd_workspace_bytes, 16-byte aligned, no
@@ -402,6 +403,17 @@ int sage_attn_bwd(const void* dout, const void* query, const void* key, const vo
                   int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
                   int64_t head_dim, const int64_t* strides, int is_causal, double sm_scale,
                   void* workspace, int64_t workspace_bytes, void* stream);
+/*
+ * The same where out and lse are what sage_attn_direct_fwd (or
+ * sage_attn_direct_fwd_vrows, _vrows_bf16, sage_attn_few_fwd with quantized 0)
+ * wrote for these very arguments: no probability exceeds 1 then, which saves
+ * the limit (1-4% of the time).  Any other lse may overflow fp16.
+ */
+int sage_attn_direct_bwd(const void* dout, const void* query, const void* key, const void* value, const void* out,
+                         const float* lse, const float* dlse, void* dq, void* dk, void* dv, int dtype,
+                         int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                         int64_t head_dim, const int64_t* strides, int is_causal, double sm_scale,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Rotary positions with several axes of one or two tensors (queries and keys;

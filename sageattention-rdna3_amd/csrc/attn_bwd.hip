@@ -167,7 +167,7 @@ __device__ __forceinline__ int ds_exponent(const BwdParams& p, int bhk, char* sm
   return __builtin_amdgcn_readfirstlane(min(max(e, -100), 100));
 }
 
-template <int D, bool BF16, bool KV>
+template <int D, bool BF16, bool CAP, bool KV>
 __device__ __forceinline__ void bwd_item(const BwdParams& p, int item, char* smem) {
   using C = BwdCfg<D>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -246,11 +246,15 @@ __device__ __forceinline__ void bwd_item(const BwdParams& p, int item, char* sme
     for (int r = 0; r < 16; ++r) own_nd[r] = nd;
   }
   float ds_scale = 1.0f;
+  [[maybe_unused]] float max_x = BF16 ? 0.0f : kF16PScale;  // CAP: exponent of P = 1
   int ds_exp = 0;
   if constexpr (!BF16) {
     ds_exp = ds_exponent(p, b * p.hkv + hk, smem);
     ds_scale = __builtin_ldexpf(1.0f, ds_exp);
-    if constexpr (!KV) own_nl += static_cast<float>(ds_exp);  // here P feeds dS alone, and takes its factor along
+    if constexpr (!KV) {  // here P feeds dS alone, and takes its factor along
+      own_nl += static_cast<float>(ds_exp);
+      max_x += static_cast<float>(ds_exp);
+    }
   }
 
   // ---- the stream.  Chunk c (16 bytes) of row r of a group of four rows lies at position 4 c + r of the group: a
@@ -376,7 +380,9 @@ __device__ __forceinline__ void bwd_item(const BwdParams& p, int item, char* sme
           nl[0] = l4.x, nl[1] = l4.y, nl[2] = l4.z, nl[3] = l4.w;
         }
       }
-      s[r] = fast_exp2(__builtin_fmaf(s[r], p.sc, KV ? nl[r % 4] : own_nl));
+      float x = __builtin_fmaf(s[r], p.sc, KV ? nl[r % 4] : own_nl);
+      if constexpr (CAP) x = __builtin_elementwise_minimum(x, max_x);  // (keeps NaN)
+      s[r] = fast_exp2(x);
       if (KV && (r & 1)) pw[r / 8][r % 8 / 2] = static_cast<int>(pack16<BF16>(s[r - 1], s[r]));
     };
     auto gradient = [&](int r) __attribute__((always_inline)) {
@@ -509,12 +515,16 @@ __device__ __forceinline__ void bwd_item(const BwdParams& p, int item, char* sme
   }
 }
 
-template <int D, bool BF16>
+// CAP: the LSE is not the one of these scores (the INT8 path's, whose scores are
+// quantised), and P = exp(S - L) can come out above 1 without a bound; it counts
+// as 1.  (The direct kernel's own LSE needs no such limit: an instruction a
+// score, 1-2% of a launch at D = 128, 3-4% at 64.)
+template <int D, bool BF16, bool CAP>
 __global__ __launch_bounds__(kBwdThreads, BwdCfg<D>::kWaves) void attn_bwd_kernel(BwdParams p) {
   __shared__ __align__(16) char smem[BwdCfg<D>::kLdsBytes];
   const int block = static_cast<int>(blockIdx.x);
-  if (block < p.kv_order.items) bwd_item<D, BF16, true>(p, item_of(block, p.kv_order), smem);
-  else bwd_item<D, BF16, false>(p, item_of(block - p.kv_order.items, p.q_order), smem);
+  if (block < p.kv_order.items) bwd_item<D, BF16, CAP, true>(p, item_of(block, p.kv_order), smem);
+  else bwd_item<D, BF16, CAP, false>(p, item_of(block - p.kv_order.items, p.q_order), smem);
 }
 
 // Row statistics: -L log2 e and -delta of kStatRows query rows a block (rows
@@ -810,30 +820,10 @@ int bwd_sizes(const char* fn, int64_t batch, int64_t q_heads, int64_t kv_heads, 
   return SAGE_OK;
 }
 
-}  // namespace
-}  // namespace sage
-
-using namespace sage;
-
-extern "C" int64_t sage_attn_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
-                                                 int64_t q_len, int64_t kv_len, int64_t head_dim, int is_causal,
-                                                 int need_dq, int need_dkv) {
-  static const char* const fn = "sage_attn_bwd_workspace_bytes";
-  clear_error();
-  if (dtype != SAGE_DTYPE_F16 && dtype != SAGE_DTYPE_BF16)
-    return set_error(SAGE_ERR_INVALID_ARG, "%s: dtype must be SAGE_DTYPE_F16 or SAGE_DTYPE_BF16, got %d", fn, dtype);
-  if (int rc = bwd_sizes(fn, batch, q_heads, kv_heads, q_len, kv_len, head_dim)) return rc;
-  if (batch == 0) return 0;
-  return bwd_plan(dtype == SAGE_DTYPE_BF16, batch, q_heads, kv_heads, q_len, kv_len, head_dim, is_causal != 0, need_dq != 0,
-                  need_dkv != 0).bytes;
-}
-
-extern "C" int sage_attn_bwd(const void* dout, const void* query, const void* key, const void* value, const void* out,
-                             const float* lse, const float* dlse, void* dq, void* dk, void* dv, int dtype,
-                             int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
-                             int64_t head_dim, const int64_t* strides, int is_causal, double sm_scale,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
-  static const char* const fn = "sage_attn_bwd";
+int attn_bwd(const char* fn, bool own_lse, const void* dout, const void* query, const void* key, const void* value,
+             const void* out, const float* lse, const float* dlse, void* dq, void* dk, void* dv, int dtype, int64_t batch,
+             int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len, int64_t head_dim, const int64_t* strides,
+             int is_causal, double sm_scale, void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   if (dtype != SAGE_DTYPE_F16 && dtype != SAGE_DTYPE_BF16)
     return set_error(SAGE_ERR_INVALID_ARG, "%s: dtype must be SAGE_DTYPE_F16 or SAGE_DTYPE_BF16, got %d", fn, dtype);
@@ -962,7 +952,9 @@ extern "C" int sage_attn_bwd(const void* dout, const void* query, const void* ke
     const dim3 rows_grid(static_cast<uint32_t>(pre));
     if (pre > 0 && (p.causal || p.sk <= kExactKeys)) attn_bwd_rows_kernel<D, BF, true><<<rows_grid, dim3(256), 0, st>>>(r);
     else if (pre > 0) attn_bwd_rows_kernel<D, BF, false><<<rows_grid, dim3(256), 0, st>>>(r);
-    attn_bwd_kernel<D, BF><<<dim3(static_cast<uint32_t>(f.kv_items + f.q_items)), dim3(kBwdThreads), 0, st>>>(p);
+    const dim3 items(static_cast<uint32_t>(f.kv_items + f.q_items));
+    if (own_lse) attn_bwd_kernel<D, BF, false><<<items, dim3(kBwdThreads), 0, st>>>(p);
+    else attn_bwd_kernel<D, BF, true><<<items, dim3(kBwdThreads), 0, st>>>(p);
     if (sum_rows > 0)
       attn_bwd_sum_kernel<D, BF><<<dim3(static_cast<uint32_t>(cdiv(sum_rows, 256 / (D / 8)))), dim3(256), 0, st>>>(
           p, static_cast<int>(kv_rows), static_cast<int>(sum_rows));
@@ -974,4 +966,39 @@ extern "C" int sage_attn_bwd(const void* dout, const void* query, const void* ke
   if (head_dim == 128) by_type(std::integral_constant<int, 128>{});
   else by_type(std::integral_constant<int, 64>{});
   return check_launch(fn);
+}
+}  // namespace
+}  // namespace sage
+
+using namespace sage;
+
+extern "C" int64_t sage_attn_bwd_workspace_bytes(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                 int64_t q_len, int64_t kv_len, int64_t head_dim, int is_causal,
+                                                 int need_dq, int need_dkv) {
+  static const char* const fn = "sage_attn_bwd_workspace_bytes";
+  clear_error();
+  if (dtype != SAGE_DTYPE_F16 && dtype != SAGE_DTYPE_BF16)
+    return set_error(SAGE_ERR_INVALID_ARG, "%s: dtype must be SAGE_DTYPE_F16 or SAGE_DTYPE_BF16, got %d", fn, dtype);
+  if (int rc = bwd_sizes(fn, batch, q_heads, kv_heads, q_len, kv_len, head_dim)) return rc;
+  if (batch == 0) return 0;
+  return bwd_plan(dtype == SAGE_DTYPE_BF16, batch, q_heads, kv_heads, q_len, kv_len, head_dim, is_causal != 0, need_dq != 0,
+                  need_dkv != 0).bytes;
+}
+
+extern "C" int sage_attn_bwd(const void* dout, const void* query, const void* key, const void* value, const void* out,
+                             const float* lse, const float* dlse, void* dq, void* dk, void* dv, int dtype,
+                             int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                             int64_t head_dim, const int64_t* strides, int is_causal, double sm_scale,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  return attn_bwd("sage_attn_bwd", false, dout, query, key, value, out, lse, dlse, dq, dk, dv, dtype, batch, q_heads,
+                  kv_heads, q_len, kv_len, head_dim, strides, is_causal, sm_scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" int sage_attn_direct_bwd(const void* dout, const void* query, const void* key, const void* value,
+                                    const void* out, const float* lse, const float* dlse, void* dq, void* dk, void* dv, int dtype,
+                                    int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                    int64_t head_dim, const int64_t* strides, int is_causal, double sm_scale,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+  return attn_bwd("sage_attn_direct_bwd", true, dout, query, key, value, out, lse, dlse, dq, dk, dv, dtype, batch, q_heads,
+                  kv_heads, q_len, kv_len, head_dim, strides, is_causal, sm_scale, workspace, workspace_bytes, stream);
 }

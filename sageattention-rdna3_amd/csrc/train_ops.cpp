@@ -60,7 +60,8 @@ struct AttnGrads {
 };
 
 AttnGrads attn_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
-                   at::Tensor dlse, int64_t layout, bool is_causal, double sm_scale, bool need_q, bool need_kv) {
+                   at::Tensor dlse, int64_t layout, bool is_causal, double sm_scale, bool need_q, bool need_kv,
+                   bool own_lse) {
   const c10::DeviceGuard guard(q.device());
   dout = rows_ready(dout, layout);
   q = rows_ready(q, layout);
@@ -89,11 +90,12 @@ AttnGrads attn_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at
     strides[3 * i + 1] = d.sh;
     strides[3 * i + 2] = d.sn;
   }
-  check_std("sage_attn_bwd",
-            sage_attn_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                          static_cast<const float*>(lse.data_ptr()), static_cast<const float*>(ptr(dlse)), ptr(g.dq),
-                          ptr(g.dk), ptr(g.dv), dtype_code(q), qd.b, qd.h, kd.h, qd.n, kd.n, qd.d, strides,
-                          is_causal ? 1 : 0, sm_scale, ws.data_ptr(), bytes, current_stream(q)));
+  check_std(own_lse ? "sage_attn_direct_bwd" : "sage_attn_bwd",
+            (own_lse ? sage_attn_direct_bwd : sage_attn_bwd)(
+                dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                static_cast<const float*>(lse.data_ptr()), static_cast<const float*>(ptr(dlse)), ptr(g.dq), ptr(g.dk),
+                ptr(g.dv), dtype_code(q), qd.b, qd.h, kd.h, qd.n, kd.n, qd.d, strides, is_causal ? 1 : 0, sm_scale,
+                ws.data_ptr(), bytes, current_stream(q)));
   return g;
 }
 
@@ -133,7 +135,7 @@ struct AttnTrain : public torch::autograd::Function<AttnTrain> {
       at::NoGradGuard no_grad;
       const auto args = ctx->saved_data["args"].toDoubleVector();
       AttnGrads g = attn_bwd(dout, s[0], s[1], s[2], s[3], s[4], grads[1], static_cast<int64_t>(args[0]),
-                             args[1] != 0.0, args[2], need_q, need_kv);
+                             args[1] != 0.0, args[2], need_q, need_kv, true);
       r[0] = g.dq;
       if (ctx->needs_input_grad(1)) r[1] = g.dk;
       if (ctx->needs_input_grad(2)) r[2] = g.dv;
@@ -315,7 +317,8 @@ py::object sageattn_backward(at::Tensor dout, at::Tensor q, at::Tensor k, at::Te
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(q.device());
   if (smooth) k = smoothed(k, layout);
-  AttnGrads g = attn_bwd(dout, q, k, v, out, lse, dlse ? *dlse : at::Tensor(), layout, is_causal, scale_or_default(sm_scale, q), true, true);
+  AttnGrads g = attn_bwd(dout, q, k, v, out, lse, dlse ? *dlse : at::Tensor(), layout, is_causal, scale_or_default(sm_scale, q), true, true,
+                         false);
   return py::make_tuple(g.dq, g.dk, g.dv);
 }
 

@@ -92,6 +92,8 @@ SIGNATURES = {
     "sage_attn_bwd_workspace_bytes": (_I64, [_I, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _I]),
     "sage_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I,
                            _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, ctypes.c_double, _P, _I64, _P]),
+    "sage_attn_direct_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I,
+                                  _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, ctypes.c_double, _P, _I64, _P]),
     "sage_rotary_axes": (_I, [_P, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _P, _I, _P, _I, _P, _P, _I, _I,
                               _P]),
     "sage_attn_workspace_bytes": (_I64, [_I, _I64, _I64, _I64, _I64, _I64, _I, _I]),

@@ -61,8 +61,9 @@ def sageattn_backward(
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv) of an attention call from its inputs, its output and its log-sum-exp, for
     programs that keep those themselves: ``out, lse = sageattn(..., return_lse=True)`` (of either
-    path; the quantised path's rounding of Q and K is then taken as the identity), or attention
-    over key ranges merged by their LSEs (pass the merged output and LSE with each range's k, v).
+    path; the quantised path's rounding of Q and K is then taken as the identity, and a probability
+    exp(score - lse) that comes out above 1 by it counts as 1), or attention over key ranges merged
+    by their LSEs (pass the merged output and LSE with each range's k, v).
 
     dout and out have q's shape, layout and dtype; lse and dlse (the LSE's gradient, optional) are
     [B,Hq,Sq] fp32.

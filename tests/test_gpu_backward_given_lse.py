@@ -107,3 +107,75 @@ def test_dead_rows_do_not_scale(d):
     dout[:, :, ::7] = 6e4
     for x, y in zip(sageattn_backward(dout, q, k, v, out, lse, dlse=dlse), want):
         assert torch.equal(x, y)
+
+
+def given(q, k, v, dout, out, lse, causal=False):
+    """Gradients of the pass's own formula in 64 bits, P = min(1, exp(S - lse)) and delta = dout out from the given output
+    and LSE, and their bounds.  Beside what ``reference`` counts, P is off by what the exponent is: S is summed in steps
+    of 16 products of fp32 (2^-20 of the sum of |q||k| scale, with its factor's rounding), the LSE and its factor 2^-22;
+    delta only by its own sum (2^-16 of the absolute one)."""
+    q, k, v, dout, out = (x.double() for x in (q, k, v, dout, out))
+    scale, g = q.shape[-1] ** -0.5, q.shape[1] // k.shape[1]
+    kk, vv = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    s = q @ kk.transpose(-1, -2) * scale
+    if causal:
+        s = s.masked_fill(torch.arange(s.shape[3], device=s.device) > torch.arange(s.shape[2], device=s.device)[:, None], float("-inf"))
+    x = s - lse.double()[..., None]
+    p = x.clamp(max=0).exp()
+    dp, delta = dout @ vv.transpose(-1, -2), (dout * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+
+    def fold(t):
+        return t.reshape(t.shape[0], k.shape[1], g, *t.shape[2:]).sum(2)
+
+    grads = dict(dq=ds @ kk * scale, dk=fold(ds.transpose(-1, -2) @ q) * scale, dv=fold(p.transpose(-1, -2) @ dout))
+
+    def bounds(dtype):
+        u, r = torch.finfo(dtype).eps / 2, 2.0 ** -16
+        tiny = 2.0 ** -39 if dtype == F16 else 0.0
+        r_p = 2.0 ** -20 * (q.abs() @ kk.abs().transpose(-1, -2)) * scale + 2.0 ** -22 * lse.double().abs()[..., None] + r
+        bound = dout.norm(dim=-1).amax() * vv.norm(dim=-1).amax() + delta.abs().amax()
+        sums = dout.abs() @ vv.abs().transpose(-1, -2) + (dout * out).abs().sum(-1, keepdim=True)
+        e_p = (u + r_p) * p + tiny
+        e_ds = (u + r_p) * ds.abs() + r * p * sums + tiny * bound
+        e = dict(dq=e_ds @ kk.abs() * scale, dk=fold(e_ds.transpose(-1, -2) @ q.abs()) * scale,
+                 dv=fold(e_p.transpose(-1, -2) @ dout.abs()))
+        least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        return {n: e[n] + (u + r) * (grads[n].abs() + e[n]) + least for n in e}
+
+    return grads, bounds, x
+
+
+@pytest.mark.parametrize("d,dtype,causal,hq,hkv", [(128, F16, False, 2, 2), (128, F16, True, 4, 2), (64, F16, False, 2, 1),
+                                                   (128, BF16, False, 2, 2), (64, BF16, True, 2, 2)])
+@pytest.mark.parametrize("std,outlier", [(2.0, 16.0), (4.0, 4.0)])
+def test_quantised_forward_with_an_outlier_channel(d, dtype, causal, hq, hkv, std, outlier, monkeypatch):
+    """One channel of Q and K is far larger than the others, as in trained models: the INT8 path's rounding of the others
+    then moves scores by whole units, and exp(score - LSE) is far above 1 for some pairs.  fp16 has no room for that."""
+    from sageattention import sageattn, sageattn_backward
+
+    for name in ("D64", "D64_CAUSAL", "D128"):
+        monkeypatch.setenv("SAGEATTN_DIRECT_THRESHOLD_" + name, "-1")
+    q, k, v, dout = inputs(1, hq, hkv, 2048, 2048, d, dtype, "HND")
+    for x in (q, k):
+        x *= std
+        x[..., 7] *= outlier
+    out, lse = sageattn(q, k, v, is_causal=causal, return_lse=True)
+    want, bounds, x = given(q, k, v, dout, out, lse, causal)
+    assert x.max() > 1.5, "no probability above 4"
+    e = bounds(dtype)
+    for name, got in zip(("dq", "dk", "dv"), sageattn_backward(dout, q, k, v, out, lse, is_causal=causal)):
+        check(got, want[name], e[name], "HND", name)
+
+
+def test_nan_lse_is_not_capped():
+    """A row whose LSE is NaN (its scores are) has NaN gradients, not those of P = 1."""
+    from sageattention import sageattn, sageattn_backward
+
+    for dtype in (F16, BF16):
+        q, k, v, dout = inputs(1, 1, 1, 90, 90, 64, dtype, "HND")
+        out, lse = sageattn(q, k, v, return_lse=True)
+        lse[0, 0, 40] = float("nan")
+        dq, dk, dv = sageattn_backward(dout, q, k, v, out, lse)
+        assert torch.isnan(dq[0, 0, 40]).all() and torch.isnan(dk).all() and torch.isnan(dv).all()
+        assert torch.isfinite(dq[0, 0, :40]).all() and torch.isfinite(dq[0, 0, 41:]).all()

@@ -535,17 +535,20 @@ __global__ __launch_bounds__(kBwdThreads, BwdCfg<D>::kWaves) void attn_bwd_kerne
 // O's rounding makes an error in delta that weighs like 1 / n in the dS of a row
 // of n keys (n = 1: dS is 0, and that error all that is left).  Rows of up to
 // kExactKeys keys take delta as the sum of P o dP instead, from two products of
-// one wave, where their P sum to 1 (an output merged from several key ranges,
-// or a quantised forward call, keeps dO O).  2-norm error of dQ over that of one
-// rounding, without / with: causal B1 H8 S64 1.59 / 1.43, S2048 1.50 / 1.44, two
-// keys 2.3 / 1.4; 2 to 4 us of a launch that has such rows.
+// one wave, where their P sum to 1 and, with a given LSE, both deltas agree
+// within half of the forward call's roundings (P to fp16, O to its type; a sum
+// over D elements stays well below them): an output merged from several key
+// ranges keeps dO O, since what its other keys add is not in the sum, however
+// small their P, and so does a quantised forward call.  2-norm error of dQ over
+// that of one rounding, without / with: causal B1 H8 S64 1.59 / 1.43, S2048 1.50
+// / 1.44, two keys 2.3 / 1.4; 2 to 4 us of a launch that has such rows.
 constexpr int kPreRows = kStatRows;
 constexpr int kExactKeys = 32;  // of an MFMA
 
 struct PreParams {
   Rows out, dout, v, q, k;
   float sc;
-  int32_t causal;
+  int32_t causal, own_lse;  // own_lse: these are all of the rows' keys
   FastDiv d_group;
   const float* lse;
   const float* dlse;  // or null
@@ -556,9 +559,10 @@ struct PreParams {
   FastDiv d_hq, d_hkv, d_heads, d_vheads;
 };
 
-// Sums of P and of P o dP of 32 rows over the first 32 keys, one wave: out[row] for the rows row0 + 0 .. 31.
+// Sums of P, P o dP and (unless own_lse) P o |dO| |V|^T of 32 rows over the first 32 keys, one wave: out[row] for the
+// rows row0 + 0 .. 31.
 template <int D, bool BF16>
-__device__ __forceinline__ void exact_sums(const PreParams& p, int b, int h, int64_t bh, int row0, float2_t* out) {
+__device__ __forceinline__ void exact_sums(const PreParams& p, int b, int h, int64_t bh, int row0, float (*out)[3]) {
   const int lane = threadIdx.x & 63, m = lane & 31, half = lane >> 5;
   const int row = row0 + m, hk = div_by(h, p.d_group);
   const bool in = row < p.sq, key_in = m < p.sk;
@@ -567,7 +571,7 @@ __device__ __forceinline__ void exact_sums(const PreParams& p, int b, int h, int
   };
   const float l = in ? p.lse[bh * p.sq + row] : -INFINITY;
   const float nl = l < kDeadLse ? -INFINITY : l * -1.4426950408889634f;
-  float16_t_ s = {}, dp = {};
+  float16_t_ s = {}, dp = {}, size = {};
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) {
     int4_t x1 = {0, 0, 0, 0}, x2 = x1, y1 = x1, y2 = x1;
@@ -575,8 +579,9 @@ __device__ __forceinline__ void exact_sums(const PreParams& p, int b, int h, int
     if (key_in) y1 = at(p.k, hk, m)[2 * t], y2 = at(p.v, hk, m)[2 * t];
     s = mfma16<BF16>(y1, x1, s);
     dp = mfma16<BF16>(y2, x2, dp);
+    if (!p.own_lse) size = mfma16<BF16>(y2 & 0x7fff7fff, x2 & 0x7fff7fff, size);
   }
-  float sum_p = 0.0f, sum = 0.0f;
+  float sum_p = 0.0f, sum = 0.0f, sum_size = 0.0f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {  // lane (m, half): row m, keys 8 (r / 4) + 4 half + r % 4
     const int key = 8 * (r >> 2) + 4 * half + (r & 3);
@@ -584,17 +589,19 @@ __device__ __forceinline__ void exact_sums(const PreParams& p, int b, int h, int
     const float pr = dead ? 0.0f : fast_exp2(__builtin_fmaf(s[r], p.sc, nl));
     sum_p += pr;
     sum += mul_legacy(pr, dp[r]);
+    sum_size += mul_legacy(pr, size[r]);
   }
   sum_p = xhalf_sum(sum_p);
   sum = xhalf_sum(sum);
-  if (half == 0) out[m] = float2_t{sum_p, sum};
+  sum_size = xhalf_sum(sum_size);
+  if (half == 0) out[m][0] = sum_p, out[m][1] = sum, out[m][2] = sum_size;
 }
 
 template <int D, bool BF16, bool FEW>
 __global__ __launch_bounds__(256) void attn_bwd_rows_kernel(PreParams p) {
   constexpr int kLanes = D / 8, kRowsPass = 256 / kLanes, kPasses = kPreRows / kRowsPass;
   __shared__ float red[2][4];
-  [[maybe_unused]] __shared__ float2_t exact[FEW ? kPreRows : 1];
+  [[maybe_unused]] __shared__ float exact[FEW ? kPreRows : 1][3];
   const int c = threadIdx.x % kLanes, r0 = threadIdx.x / kLanes;
   const bool is_v = static_cast<int>(blockIdx.x) >= p.q_total;
   // query blocks: the first of every head, then the second, ...: those with few keys take longest
@@ -648,9 +655,10 @@ __global__ __launch_bounds__(256) void attn_bwd_rows_kernel(PreParams p) {
       if constexpr (!BF16) sq += __shfl_xor(sq, s);
     }
     if (few && (all || x * kRowsPass + r0 < 32)) {
-      const float2_t e = exact[x * kRowsPass + r0];
-      // what P lack of 1 may belong to keys elsewhere: below 2^-14 it weighs less than O's rounding in either type
-      if (__builtin_fabsf(e.x - 1.0f) <= 0x1p-14f) dot = e.y;
+      const float(&e)[3] = exact[x * kRowsPass + r0];
+      constexpr float kRounding = 0x1p-11f + (BF16 ? 0x1p-9f : 0x1p-11f);  // of the forward call, times e[2]
+      const bool whole = p.own_lse || __builtin_fabsf(e[1] - dot) <= 0.5f * kRounding * e[2];
+      if (whole && __builtin_fabsf(e[0] - 1.0f) <= 0x1p-14f) dot = e[1];
     }
     // a row without a live key: P = 0 everywhere, and its (arbitrary) delta must not meet it as NaN
     const bool live = is_v || (row < n && !(wl[x] < kDeadLse));
@@ -922,6 +930,7 @@ int attn_bwd(const char* fn, bool own_lse, const void* dout, const void* query, 
   r.k = rows[2];
   r.sc = p.sc;
   r.causal = p.causal;
+  r.own_lse = own_lse;
   r.d_group = p.d_group;
   r.lse = lse;
   r.dlse = dlse;

@@ -179,3 +179,32 @@ def test_nan_lse_is_not_capped():
         dq, dk, dv = sageattn_backward(dout, q, k, v, out, lse)
         assert torch.isnan(dq[0, 0, 40]).all() and torch.isnan(dk).all() and torch.isnan(dv).all()
         assert torch.isfinite(dq[0, 0, :40]).all() and torch.isfinite(dq[0, 0, 41:]).all()
+
+
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16), (128, F16)])
+@pytest.mark.parametrize("far", [40.0, 1000.0, 20000.0])
+@pytest.mark.parametrize("n", [3, 20, 32])
+def test_few_keys_of_a_merged_range(d, dtype, far, n):
+    """A row's keys but for 2^-15 of its weight are a range of at most 32, whose P sum to 1 as nearly as fp32 tells.  The
+    other keys' V is far larger: delta has to keep their part, which the range's own sum lacks."""
+    q, k, v, dout = inputs(1, 2, 2, 150, n + 40, d, dtype, "HND", seed=12)
+    q[..., 0], k[..., 0] = 1, 0
+    k[:, :, n:] *= 0.25
+    k[:, :, n:, 0] = -14.0 * d ** 0.5
+    v[:, :, n:] *= far / 4
+    merged(q, k, v, dout, (slice(0, n), slice(n, n + 40)), dtype)
+
+
+@pytest.mark.parametrize("b,h,sq,sk,causal", [(1, 8, 64, 64, True), (1, 4, 131, 131, True), (2, 4, 200, 2, False), (1, 8, 300, 31, False)])
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16), (64, BF16), (128, F16)])
+def test_few_keys_of_a_whole_call(b, h, sq, sk, causal, d, dtype):
+    """With the LSE of a call over these very keys, rows of few keys take delta from their probabilities as the autograd
+    node does: the same bits."""
+    from sageattention import sageattn_backward, sageattn_train
+
+    q, k, v, dout = inputs(b, h, h, sq, sk, d, dtype, "HND", seed=8)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out, lse = sageattn_train(*leaves, is_causal=causal, return_lse=True)
+    want = torch.autograd.grad(out, leaves, dout)
+    got = sageattn_backward(dout, *(x.detach() for x in leaves), out.detach(), lse.detach(), is_causal=causal)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

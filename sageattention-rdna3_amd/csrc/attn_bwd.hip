@@ -444,12 +444,11 @@ __device__ __forceinline__ void bwd_item(const BwdParams& p, int item, char* sme
     if (i < n) issue(i);
   int slot = 0;
   for (int i = 0; i < n; ++i) {
-    // loads of the stages after this one may stay in flight
+    // loads of the stage after this one may stay in flight
+    static_assert(kFly <= 2, "one later stage at most");
     constexpr int kV = 2 * kLoadsWave;
-    const int later = min(kFly - 1, n - 1 - i);
-    if (later == 0) bwd_wait_vm<0>();
-    else if (later == 1) KV && wave == 0 ? bwd_wait_vm<kV + 1>() : bwd_wait_vm<kV>();
-    else KV && wave == 0 ? bwd_wait_vm<2 * kV + 2>() : bwd_wait_vm<2 * kV>();
+    if (kFly == 1 || i == n - 1) bwd_wait_vm<0>();
+    else KV && wave == 0 ? bwd_wait_vm<kV + 1>() : bwd_wait_vm<kV>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");  // no LDS read of the stage moves above the barrier
     if (i + kFly < n) issue(slot == 0 ? C::kSlots - 1 : slot - 1);

@@ -55,6 +55,8 @@ int dtype_code(const at::Tensor& t) {
 // A contiguous gradient in the layout of `like` (whose own strides may be those of a view or an expanded tensor).
 at::Tensor grad_like(const at::Tensor& like) { return at::empty(like.sizes(), like.options()); }
 
+bool dual(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 struct AttnGrads {
   at::Tensor dq, dk, dv;
 };
@@ -130,6 +132,7 @@ struct AttnTrain : public torch::autograd::Function<AttnTrain> {
     const bool need_q = ctx->needs_input_grad(0), need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     variable_list r(6);
     if (!grads[0].defined() && !grads[1].defined()) return r;
+    if (dual(grads[0]) || dual(grads[1])) throw std::runtime_error("sageattn_train has no forward-mode derivative");
     at::Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(s[3]);
     {
       at::NoGradGuard no_grad;
@@ -238,6 +241,15 @@ void require_value(bool ok, const std::string& message) {
   if (!ok) throw py::value_error(message);
 }
 
+// A dual tensor need not require grad, and its tangent would be lost without a word.
+void refuse_dual(const char* fn, std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors) {
+    if (t == nullptr || !dual(*t)) continue;
+    PyErr_SetString(PyExc_NotImplementedError, (std::string(fn) + " has no forward-mode derivative").c_str());
+    throw py::error_already_set();
+  }
+}
+
 int64_t layout_code(const py::handle& name) {
   if (py::isinstance<py::str>(name)) {
     const std::string s = py::cast<std::string>(name);
@@ -273,6 +285,7 @@ py::object sageattn_train(at::Tensor q, at::Tensor k, at::Tensor v, const py::ob
                           std::optional<double> sm_scale, bool return_lse) {
   const int64_t layout = layout_code(tensor_layout);
   check_qkv(q, k, v, layout);
+  refuse_dual("sageattn_train", {&q, &k, &v});
   const c10::DeviceGuard guard(q.device());
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
     auto r = attn_fwd(q, k, v, layout, is_causal, scale_or_default(sm_scale, q), return_lse, false, true, 0, current_stream(q));
@@ -313,6 +326,7 @@ py::object sageattn_backward(at::Tensor dout, at::Tensor q, at::Tensor k, at::Te
     require_value(t == nullptr || (t->sizes() == at::IntArrayRef(rows) && t->scalar_type() == at::kFloat && t->device() == q.device()),
                   std::string(name) + " must be [" + std::to_string(d.b) + ", " + std::to_string(d.h) + ", " +
                       std::to_string(d.n) + "] fp32 on the device of q");
+  refuse_dual("sageattn_backward", {&dout, &q, &k, &v, &out, &lse, optional_dlse});
   require_value(!smooth || dlse == std::nullopt, "dlse is not taken with smooth_k=True");
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(q.device());
@@ -358,6 +372,7 @@ py::object rotary_axes(at::Tensor q, const std::optional<at::Tensor>& k, at::Ten
   require_value(positions.sizes() == at::IntArrayRef({n, na}) || positions.sizes() == at::IntArrayRef({b, n, na}),
                 "positions must be [" + std::to_string(n) + ", " + std::to_string(na) + "] or [" + std::to_string(b) +
                     ", " + std::to_string(n) + ", " + std::to_string(na) + "], got " + shape_str(positions));
+  refuse_dual("rotary_axes", {&q, k ? &*k : nullptr, &positions});
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k && k->requires_grad()))) {  // no node: ~2 us
     variable_list r = rotate(q, k ? *k : at::Tensor(), positions, c);
     if (!k) return py::cast(r[0]);

@@ -33,8 +33,8 @@ def sageattn_train(
     ``sageattn``; fp16 or bf16, head_dim 64 or 128.  Saved for the backward pass: q, k, v, the
     output and the LSE.  With ``return_lse`` the LSE ([B,Hq,Sq] fp32) is returned too, and its
     gradient is taken into account.  Gradients are deterministic (no atomics); dk and dv sum over
-    the query heads that share a kv head.  They cannot be differentiated a second time (asking for
-    it raises).
+    the query heads that share a kv head.  They cannot be differentiated a second time, and there are
+    no forward-mode derivatives (asking for either raises).
 
     A row without a live key (all its scores -inf) gets output 0, LSE -inf and zero gradients.  The
     backward pass takes exp(score - LSE) in fp32, which is off by about 2^-22 |LSE| of itself: scores
@@ -92,7 +92,7 @@ def rotary_axes(
 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Rotary positions with several axes (an image's height and width, a video's time, height and
     width, one axis for text), of queries and keys in one launch; differentiable, any number of
-    times, in q and k.
+    times, in q and k (not in forward mode, which raises).
 
     q: [B,Hq,N,D] (HND) or [B,N,Hq,D] (NHD), fp16, bf16 or fp32, D 64 or 128; k likewise with its
     own head count, or None (then one tensor is returned).  positions: [N, A] or [B, N, A], int32,

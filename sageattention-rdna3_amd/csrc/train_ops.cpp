@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <vector>
@@ -52,8 +53,36 @@ int dtype_code(const at::Tensor& t) {
   }
 }
 
-// A contiguous gradient in the layout of `like` (whose own strides may be those of a view or an expanded tensor).
-at::Tensor grad_like(const at::Tensor& like) { return at::empty(like.sizes(), like.options()); }
+// The kernels' byte offsets within a head are 32-bit, up to 128 rows past its end (sage_attn_bwd).
+bool head_fits(int64_t n, int64_t sn) { return (n + 128) * sn * 2 <= static_cast<int64_t>(UINT32_MAX); }
+
+// rows_ready, with every head's rows within those offsets: [B,N,H,D] of many heads and tokens is copied head by head.
+at::Tensor heads_ready(const at::Tensor& t, int64_t layout) {
+  const at::Tensor r = rows_ready(t, layout);
+  const Dims d = bhnd(r, layout);
+  if (d.n <= 1 || head_fits(d.n, d.sn)) return r;
+  return layout == 1 ? r.clone(at::MemoryFormat::Contiguous) : r.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
+}
+
+// A gradient in the layout of `like` (whose own strides may be those of a view or an expanded tensor): contiguous, or head
+// by head where heads_ready would copy it.
+at::Tensor grad_like(const at::Tensor& like, int64_t layout) {
+  const Dims d = bhnd(like, layout);
+  if (layout == 1 || head_fits(d.n, d.h * d.d)) return at::empty(like.sizes(), like.options());
+  return at::empty({d.b, d.h, d.n, d.d}, like.options()).transpose(1, 2);
+}
+
+// The backward pass's limits, told by the forward call (they start near 2^24 tokens, or 2^24 blocks of 64).
+void check_bwd_sizes(const at::Tensor& q, const at::Tensor& k, int64_t layout, bool is_causal) {
+  const Dims a = bhnd(q, layout), b = bhnd(k, layout);
+  constexpr int64_t kMany = 1 << 24;
+  if (a.n < kMany - 128 && b.n < kMany - 128 && a.b * a.h < kMany && a.b * a.h * ((a.n + 63) / 64 + (b.n + 63) / 64) < kMany) return;
+  const int64_t rc = sage_attn_bwd_workspace_bytes(dtype_code(q), a.b, a.h, b.h, a.n, b.n, a.d, is_causal ? 1 : 0, 1, 1);
+  if (rc < 0) check("sage_attn_bwd_workspace_bytes", static_cast<int>(rc));
+  if (!head_fits(std::max(a.n, b.n), a.d))
+    throw py::value_error("sageattn_train: the backward pass takes heads of up to " +
+                          std::to_string(UINT32_MAX / (2 * a.d) - 128) + " tokens");
+}
 
 bool dual(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 
@@ -65,18 +94,18 @@ AttnGrads attn_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at
                    at::Tensor dlse, int64_t layout, bool is_causal, double sm_scale, bool need_q, bool need_kv,
                    bool own_lse) {
   const c10::DeviceGuard guard(q.device());
-  dout = rows_ready(dout, layout);
-  q = rows_ready(q, layout);
-  k = rows_ready(k, layout);
-  v = rows_ready(v, layout);
-  out = rows_ready(out, layout);
+  dout = heads_ready(dout, layout);
+  q = heads_ready(q, layout);
+  k = heads_ready(k, layout);
+  v = heads_ready(v, layout);
+  out = heads_ready(out, layout);
   lse = lse.contiguous();
   if (dlse.defined()) dlse = dlse.contiguous();
   AttnGrads g;
-  if (need_q) g.dq = grad_like(q);
+  if (need_q) g.dq = grad_like(q, layout);
   if (need_kv) {
-    g.dk = grad_like(k);
-    g.dv = grad_like(v);
+    g.dk = grad_like(k, layout);
+    g.dv = grad_like(v, layout);
   }
   const Dims qd = bhnd(q, layout), kd = bhnd(k, layout);
   const int64_t bytes = sage_attn_bwd_workspace_bytes(dtype_code(q), qd.b, qd.h, kd.h, qd.n, kd.n, qd.d, is_causal ? 1 : 0,
@@ -292,6 +321,7 @@ py::object sageattn_train(at::Tensor q, at::Tensor k, at::Tensor v, const py::ob
     if (return_lse) return py::make_tuple(r.first, r.second);
     return py::cast(r.first);
   }
+  check_bwd_sizes(q, k, layout, is_causal);
   variable_list r = AttnTrain::apply(q, k, v, layout, is_causal, scale_or_default(sm_scale, q));
   if (return_lse) return py::make_tuple(r[0], r[1]);
   return py::cast(r[0]);

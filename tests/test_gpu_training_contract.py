@@ -37,3 +37,43 @@ def test_forward_mode_is_refused():
             torch.autograd.grad(rotary_axes(leaf, None, pos, [64]), leaf, dd)
         plain = sageattn_train(q, k, v)
     assert torch.equal(plain, out)
+
+
+@pytest.mark.parametrize("shape_q,shape_k", [((1, 1, 2 ** 24 - 127, 128), (1, 1, 64, 128)), ((1, 1, 64, 128), (1, 1, 2 ** 24, 128)),
+                                             ((1, 1, 2 ** 25, 64), (1, 1, 64, 64)), ((4, 2 ** 14, 2 ** 15, 64), (4, 2 ** 14, 64, 64)),
+                                             ((2 ** 24, 1, 64, 64), (2 ** 24, 1, 64, 64)), ((1, 1, 2 ** 31, 64), (1, 1, 64, 64))])
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_limits_are_told_by_the_forward_call(shape_q, shape_k, layout):
+    """Sizes that the backward pass does not take.  (Expanded tensors: no memory, and no kernel reads them.)"""
+    from sageattention import sageattn_train
+    from sageattention._capi import SageError
+
+    def make(shape):
+        x = torch.zeros(1, 1, 1, shape[3], dtype=BF16, device="cuda").requires_grad_(True).expand(shape)
+        return x.transpose(1, 2) if layout == "NHD" else x
+
+    q, k = make(shape_q), make(shape_k)
+    before = torch.cuda.memory_allocated()
+    with pytest.raises((SageError, ValueError), match="limits|tokens"):
+        sageattn_train(q, k, k, tensor_layout=layout)
+    assert torch.cuda.memory_allocated() == before
+
+
+def test_many_heads_of_many_tokens():
+    """[B,N,H,D] whose heads span more than 32-bit offsets, in q, the output and their gradients: the gradients of the
+    same call head by head, bit for bit."""
+    from sageattention import sageattn_train
+
+    b, h, n, d = 1, 64, 262144, 128
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, dout = (torch.randn(b, n, h, d, generator=g, device="cuda", dtype=BF16) for _ in range(2))
+    k, v = (torch.randn(b, 50, h, d, generator=g, device="cuda", dtype=BF16) for _ in range(2))
+
+    def grads(layout):
+        turn = (lambda x: x) if layout == "NHD" else (lambda x: x.transpose(1, 2).contiguous())
+        leaves = [turn(x).requires_grad_(True) for x in (q, k, v)]
+        out = sageattn_train(*leaves, tensor_layout=layout)
+        return [x if layout == "NHD" else x.transpose(1, 2) for x in (out.detach(), *torch.autograd.grad(out, leaves, turn(dout)))]
+
+    for x, y in zip(grads("NHD"), grads("HND")):
+        assert x.shape == y.shape and torch.equal(x, y)

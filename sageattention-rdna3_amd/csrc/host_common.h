@@ -45,12 +45,13 @@ inline Dims bhnd(const at::Tensor& t, int64_t layout) {
 }
 
 // t, or a copy that meets the 16-byte access contract (16-byte aligned base,
-// batch/head/token strides multiples of 8 elements)
+// batch/head/token strides multiples of 8 elements; a plain clone would keep
+// the odd stride of a dimension of one element)
 inline at::Tensor vector_ready(const at::Tensor& t) {
   const auto st = t.strides();
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0)
     return t;
-  return t.is_contiguous() ? t.clone() : t.contiguous();
+  return t.clone(at::MemoryFormat::Contiguous);
 }
 
 inline std::string shape_str(const at::Tensor& t) {

@@ -42,7 +42,7 @@ at::Tensor rows_ready(const at::Tensor& t, int64_t layout) {
   if (t.stride(3) == 1 && (d.n <= 1 || d.sn >= d.d) && d.sb % align == 0 && d.sh % align == 0 && d.sn % align == 0 &&
       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
     return t;
-  return t.is_contiguous() ? t.clone() : t.contiguous();
+  return t.clone(at::MemoryFormat::Contiguous);
 }
 
 int dtype_code(const at::Tensor& t) {

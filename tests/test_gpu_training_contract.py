@@ -77,3 +77,35 @@ def test_many_heads_of_many_tokens():
 
     for x, y in zip(grads("NHD"), grads("HND")):
         assert x.shape == y.shape and torch.equal(x, y)
+
+
+def one_token_slices(heads, d, dtype, layout, odd):
+    """q, k, v and an output gradient of one token: slices of rows whose length is odd, so that the strides of the batch
+    and token dimensions, of one element each, are odd too."""
+    g = torch.Generator().manual_seed(4)
+    row = torch.nn.functional.pad(torch.randn(1, 1, 4 * heads * d, generator=g), (0, odd)).to(dtype).cuda()
+    out = [row[..., i * heads * d:(i + 1) * heads * d].reshape(1, 1, heads, d) if not odd else
+           row[..., i * heads * d:(i + 1) * heads * d].as_strided((1, 1, heads, d), (row.shape[2], row.shape[2], d, 1), i * heads * d)
+           for i in range(4)]
+    return [x if layout == "NHD" else x.transpose(1, 2) for x in out]
+
+
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+@pytest.mark.parametrize("odd", [1, 4])
+def test_odd_strides_of_dimensions_of_one(layout, odd):
+    from sageattention import rotary_axes, sageattn, sageattn_backward, sageattn_train
+
+    def results(odd):
+        q, k, v, dout = one_token_slices(4, 64, BF16, layout, odd)
+        pos = torch.full((1, 1), 7, device="cuda")
+        outs = list(rotary_axes(q, k, pos, [64], tensor_layout=layout))
+        even = q.clone(memory_format=torch.contiguous_format)  # sageattn refuses odd strides of q, as the reference does
+        outs.append(sageattn(even, k, v, tensor_layout=layout))
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out, lse = sageattn_train(*leaves, tensor_layout=layout, return_lse=True)
+        outs += [out.detach(), lse.detach(), *torch.autograd.grad(out, leaves, dout)]
+        outs += sageattn_backward(dout, q, k, v, out.detach(), lse.detach(), tensor_layout=layout)
+        return outs
+
+    for x, y in zip(results(odd), results(0)):
+        assert torch.equal(x, y)

@@ -229,9 +229,13 @@ struct RotaryAxes : public torch::autograd::Function<RotaryAxes> {
     args.insert(args.end(), c.axes.begin(), c.axes.end());
     ctx->saved_data["args"] = std::move(args);
     ctx->set_materialize_grads(false);
-    variable_list made;
-    for (auto& o : out)
-      if (o.defined()) made.push_back(o);
+    variable_list made, fixed;
+    for (int i = 0; i < 2; ++i) {
+      if (!out[i].defined()) continue;
+      made.push_back(out[i]);
+      if (!(i == 0 ? q : k)->requires_grad()) fixed.push_back(out[i]);
+    }
+    ctx->mark_non_differentiable(fixed);  // of an input without a gradient: attention then computes none for it either
     return made;
   }
 

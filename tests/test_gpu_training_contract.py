@@ -109,3 +109,23 @@ def test_odd_strides_of_dimensions_of_one(layout, odd):
 
     for x, y in zip(results(odd), results(0)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("frozen", ["q", "k"])
+def test_rotary_of_an_input_without_gradient(frozen):
+    """The turned q or k of an input that needs no gradient needs none itself; the other's gradient is the same."""
+    from sageattention import rotary_axes
+
+    q, k, _, _ = inputs(1, 4, 2, 50, 50, 64, F32, "HND")
+    pos = torch.arange(50, device="cuda")[:, None]
+    both = [x.clone().requires_grad_(True) for x in (q, k)]
+    outs = rotary_axes(*both, pos, [64])
+    weights = [torch.randn_like(x) for x in outs]
+    want = torch.autograd.grad(outs, both, weights, create_graph=True)
+    assert all(x.requires_grad for x in outs)
+    one = [x.clone().requires_grad_(name != frozen) for name, x in (("q", q), ("k", k))]
+    turned = rotary_axes(*one, pos, [64])
+    assert [x.requires_grad for x in turned] == [frozen != "q", frozen != "k"]
+    i = 1 if frozen == "q" else 0
+    got = torch.autograd.grad(turned[i], one[i], weights[i])[0]
+    assert torch.equal(got, want[i]) and torch.equal(turned[i], outs[i]) and torch.equal(turned[1 - i], outs[1 - i])

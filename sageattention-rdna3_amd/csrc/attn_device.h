@@ -109,14 +109,23 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 // largest key's may miss 0 by the rounding of the max itself: at most a half
 // below 2^24, but up to 2^100 where keys are masked with the lowest value of a
 // type, either way (P infinite, or 0 for every key).  Rows with a reference max
-// from 2^24 on round the score like the max instead (huge_score), which makes
-// that difference 0 and every other one negative; the score's own fp32 sum is
-// off by as much.  Such a row's max moves with every tile (a step of it is more
-// than the lazy threshold), so it is never behind a score.  (-FLT_MAX is a row
-// without a live key so far.)
+// from 2^24 on (huge_ref; -FLT_MAX is a row without a live key so far) therefore
+// take a form whose product is exact or rounded like the max, so that the largest
+// key's difference is 0.  One scale for all keys (direct kinds): the power of two
+// below it, in the product and in the row's max (huge_scale).  Differences of
+// scores are then down to half as large, but they are those of fp32 sums whose
+// steps are 1 or more; the LSE takes the max back to the scale (unscaled_max).
+// Otherwise: the score is rounded before the max is subtracted (huge_score).
 __device__ __forceinline__ bool huge_ref(float m) {
-  const float a = __builtin_fabsf(m);
-  return a >= 0x1p24f && a < FLT_MAX;
+  // 2^24 <= |m| < FLT_MAX, in integers (their literals need no scalar registers, which the attention kernels spill)
+  return (__float_as_uint(m) & 0x7fffffffu) - 0x4b800000u < 0x7f7fffffu - 0x4b800000u;
+}
+__device__ __forceinline__ float huge_scale(float sc) {
+  return __uint_as_float(__float_as_uint(sc) & 0x7f800000u);
+}
+// rsc: the row's scale, sc or huge_scale(sc)
+__device__ __forceinline__ float unscaled_max(float m, float rsc, float sc) {
+  return rsc == sc ? m : m * __builtin_amdgcn_rcpf(rsc) * sc;
 }
 __device__ __forceinline__ float huge_score(float x, float sc, float m) {
 #pragma clang fp contract(off)

@@ -30,14 +30,14 @@ def make(sq, sk, d, dtype, a, b, second=None):
     return [x.to(dtype).cuda() for x in (q, k, v)] + [top.cuda()]
 
 
-def check(o, lse, q, k, v, weights, path="direct"):
+def check(o, lse, q, k, v, weights, path="direct", scale=None):
     """weights [sq, sk]: 1 for the keys of a row's largest score, else 0."""
     w = weights.double()
     n = w.sum(-1, keepdim=True)
     want, size = w @ v.double() / n, w @ v.double().abs() / n
     off = (o.double() - want).abs()
     assert (off <= (torch.finfo(o.dtype).eps / 2 + 2.0 ** -20) * want.abs() + (2.0 ** -11 + 2.0 ** -14) * size).all(), off.max().item()
-    s = (q.double()[..., :1] @ k.double()[..., :1].transpose(-1, -2)).masked_fill(w == 0, float("-inf")).amax(-1) * q.shape[-1] ** -0.5
+    s = (q.double()[..., :1] @ k.double()[..., :1].transpose(-1, -2)).masked_fill(w == 0, float("-inf")).amax(-1) * (scale or q.shape[-1] ** -0.5)
     want_lse = s + n[..., 0].log()
     assert ((lse.double() - want_lse).abs() <= (4 if path == "direct" else 22) * 2.0 ** -24 * want_lse.abs() + 1e-5).all()
 
@@ -133,3 +133,26 @@ def test_left_padded_causal(value, d):
     for o, lse in (sageattn(q, k, v, is_causal=True, return_lse=True),
                    sageattn_train(q.requires_grad_(True), k, v, is_causal=True, return_lse=True)):
         check(o[:, :, :pad].detach(), lse[:, :, :pad].detach(), q[:, :, :pad].detach(), k[:, :, :pad], v[:, :, :pad], w)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("order", ["low first", "high first", "mixed"])
+@pytest.mark.parametrize("path", ["direct", "int8"])
+@pytest.mark.parametrize("sq,d", [(1, 64), (600, 64), (600, 128)])
+def test_scores_on_both_sides_of_the_line(sign, order, path, sq, d, monkeypatch):
+    """Scores just below and just above 2^24 in log2 units, where a row's form changes (the two differ by thousands, so the
+    larger ones have all the weight)."""
+    from sageattention import sageattn
+
+    if path == "int8":
+        int8(monkeypatch)
+    sk, values = 416, torch.tensor([1.155e7, 1.17e7]).to(BF16)
+    assert values[0].item() * 1.4427 < 2 ** 24 < values[1].item() * 1.4427
+    q, k, v, _ = make(sq, sk, d, BF16, 1.0, 0.0)
+    i = torch.arange(sk)
+    high = {"low first": i >= 208, "high first": i < 208, "mixed": i // 16 % 3 == 1}[order]
+    k[..., 0] = torch.where(high, values[1], values[0]).cuda() * sign
+    top = (high if sign > 0 else ~high).cuda()
+    o, lse = sageattn(q, k, v, sm_scale=1.0, return_lse=True)
+    w = top.expand(sq, sk)
+    check(o, lse, q, k, v, w, path, 1.0)

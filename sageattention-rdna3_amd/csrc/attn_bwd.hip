@@ -886,7 +886,7 @@ int attn_bwd(const char* fn, bool own_lse, const void* dout, const void* query, 
   p.part = reinterpret_cast<float*>(ws + f.part_off);
   p.sm_scale = static_cast<float>(sm_scale);
   p.sc = p.sm_scale * 1.4426950408889634f;
-  if (p.sc == 0.0f) p.sc = 1e-38f;  // a dead pair's infinite S stays infinite
+  if (p.sc == 0.0f) p.sc = 0x1p-126f;  // a dead pair's infinite S stays infinite
   p.hq = static_cast<int32_t>(q_heads);
   p.hkv = static_cast<int32_t>(kv_heads);
   p.group = static_cast<int32_t>(q_heads / kv_heads);

@@ -129,3 +129,28 @@ def test_rotary_of_an_input_without_gradient(frozen):
     i = 1 if frozen == "q" else 0
     got = torch.autograd.grad(turned[i], one[i], weights[i])[0]
     assert torch.equal(got, want[i]) and torch.equal(turned[i], outs[i]) and torch.equal(turned[1 - i], outs[1 - i])
+
+
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_rows_far_apart(layout):
+    """Two tokens 32 MB apart in q, v and the output's gradient: past the kernels' 32-bit offsets (which run 128 rows past
+    the end), so they are copied."""
+    from sageattention import sageattn_train
+
+    g = torch.Generator().manual_seed(6)
+    near = [torch.randn(1, 3, 2, 64, generator=g).to(BF16).cuda() for _ in range(4)]
+    far = []
+    for x in near:
+        y = torch.zeros(2 ** 24 + 3 * 64, dtype=BF16, device="cuda").as_strided((1, 3, 2, 64), (2 ** 25, 64, 2 ** 24, 1))
+        y.copy_(x)
+        far.append(y)
+    far[1] = near[1]  # the forward call refuses such a k
+
+    def grads(tensors):
+        q, k, v, dout = (x if layout == "HND" else x.transpose(1, 2) for x in tensors)
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = sageattn_train(*leaves, tensor_layout=layout)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    for x, y in zip(grads(far), grads(near)):
+        assert torch.equal(x, y)

@@ -39,8 +39,8 @@ def sageattn_train(
     A row without a live key (all its scores -inf) gets output 0, LSE -inf and zero gradients.  The
     backward pass takes exp(score - LSE) in fp32, which is off by about 2^-22 |LSE| of itself: scores
     beyond some 10^4 cost precision, and from 2^21 on it means nothing.  A row whose LSE is below
-    -2^21 (all its keys masked by a large finite value; the output is their mean) has zero gradients,
-    scores above 2^21 are outside the range.  K and V have to be finite, masked or not, and bf16 V
+    -2^21 (all its keys masked by a large finite value; the output is their mean, or with key splits
+    that of the splits' by LSEs of fp32) has zero gradients, scores above 2^21 are outside the range.  K and V have to be finite, masked or not, and bf16 V
     within fp16's range (65504), as the forward kernel takes it.
     """
     return core._host().sageattn_train(q, k, v, tensor_layout, is_causal, sm_scale, return_lse)
@@ -100,7 +100,7 @@ def rotary_axes(
     widths, their sum R at most D.  Pair j of axis a turns by positions[a] * theta_a^(-2j/axes_dim[a]),
     (x, y) -> (x cos - y sin, x sin + y cos); theta is one number or one per axis.  The pairs, counted
     through the axes in order, are elements (2i, 2i+1) when ``interleaved``, else (i, i + R/2).
-    Elements past R are copied.  ``inverse`` turns the other way.  Angles are reduced in 64 bits, so
-    far positions are exact; the rotation is fp32, rounded once.
+    Elements past R are copied.  ``inverse`` turns the other way.  Angles are reduced in 64 bits and off by
+    about 2^-50 of themselves (int64 positions are taken to fp64); the rotation is fp32, rounded once.
     """
     return core._host().rotary_axes(q, k, positions, axes_dim, theta, tensor_layout, interleaved, inverse)

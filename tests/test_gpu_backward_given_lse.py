@@ -208,3 +208,62 @@ def test_few_keys_of_a_whole_call(b, h, sq, sk, causal, d, dtype):
     want = torch.autograd.grad(out, leaves, dout)
     got = sageattn_backward(dout, *(x.detach() for x in leaves), out.detach(), lse.detach(), is_causal=causal)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_merges(seed):
+    """Random range borders, scales of each range's K and V, shared heads, and a gradient of the LSE."""
+    from sageattention import sageattn_backward, sageattn_train
+
+    g = torch.Generator().manual_seed(100 + seed)
+
+    def pick(*options):
+        return options[torch.randint(len(options), (1,), generator=g).item()]
+
+    d, dtype, group = pick(64, 128), pick(F16, BF16, F16), pick(1, 2, 4)
+    hkv, sq = pick(1, 2, 3), pick(1, 31, 100, 300)
+    sizes = [pick(1, 5, 32, 33, 100, 260) for _ in range(pick(2, 3))]
+    q, k, v, dout = inputs(pick(1, 2), hkv * group, hkv, sq, sum(sizes), d, dtype, "HND", seed=seed, dout_scale=pick(1e-3, 1.0, 30.0))
+    ranges, at = [], 0
+    for n in sizes:
+        r = slice(at, at + n)
+        k[:, :, r] *= pick(0.1, 1.0, 2.0)
+        v[:, :, r] *= pick(0.0, 1e-3, 1.0, 100.0)
+        ranges.append(r)
+        at += n
+    out, lse = sageattn_train(q, k, v, return_lse=True)
+    dlse = torch.randn(lse.shape, generator=g).cuda() * pick(0.0, 1.0, 1000.0)
+    want, bounds = reference(q, k, v, dout, "HND", False, dlse=dlse)
+    e = bounds(dtype)
+    parts = [sageattn_backward(dout, q, k[:, :, r], v[:, :, r], out, lse, dlse=dlse) for r in ranges]
+    for i, name in ((1, "dk"), (2, "dv")):
+        check(torch.cat([p[i] for p in parts], 2), want[name], e[name], "HND", name)
+    dq = [p[0].double() for p in parts]
+    check(sum(dq), want["dq"], e["dq"] + torch.finfo(dtype).eps / 2 * sum(x.abs() for x in dq), "HND", "dq")
+
+
+def test_captured_and_replayed():
+    """The functional form in a graph, with smoothing and a NaN-free output, replayed with eager work between; two graphs
+    of other sizes one after the other."""
+    from sageattention import sageattn, sageattn_backward
+
+    for s, dtype in ((2304, BF16), (2100, F16)):
+        q, k, v, dout = inputs(1, 2, 1, s, s, 128, dtype, "HND")
+        out, lse = sageattn(q, k, v, smooth_k=True, return_lse=True)
+        ref = sageattn_backward(dout, q, k, v, out, lse, smooth_k=True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            sageattn_backward(dout, q, k, v, out, lse, smooth_k=True)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = sageattn_backward(dout, q, k, v, out, lse, smooth_k=True)
+        for _ in range(3):
+            for x in got:
+                x.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            again = sageattn_backward(dout, q, k, v, out, lse, smooth_k=True)
+            assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(got, ref, again))

@@ -42,9 +42,9 @@ def check(o, lse, q, k, v, weights, path="direct", scale=None):
     assert ((lse.double() - want_lse).abs() <= (4 if path == "direct" else 22) * 2.0 ** -24 * want_lse.abs() + 1e-5).all()
 
 
-def int8(monkeypatch):
+def int8(monkeypatch, longest_direct=-1):
     for name in ("D64", "D64_CAUSAL", "D64_CROSS", "D128", "D128_CROSS"):
-        monkeypatch.setenv("SAGEATTN_DIRECT_THRESHOLD_" + name, "-1")
+        monkeypatch.setenv("SAGEATTN_DIRECT_THRESHOLD_" + name, str(longest_direct))
 
 
 @pytest.mark.parametrize("dtype,a,b", SCORES)
@@ -156,3 +156,24 @@ def test_scores_on_both_sides_of_the_line(sign, order, path, sq, d, monkeypatch)
     o, lse = sageattn(q, k, v, sm_scale=1.0, return_lse=True)
     w = top.expand(sq, sk)
     check(o, lse, q, k, v, w, path, 1.0)
+
+
+@pytest.mark.parametrize("a,b", [(1.0, -1e9), (1.0, 5e9), (1.0, LOWEST)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("path", ["direct", "int8"])
+@pytest.mark.parametrize("sq,sk,causal", [(200, 2300, False), (300, 4500, False), (2300, 2300, True), (130, 1100, False)])
+def test_equal_scores_of_many_keys(a, b, d, path, sq, sk, causal, monkeypatch):
+    """Many key tiles of a wave (the pipelined steps), two key groups of a block.  Unsplit: a split's LSE does not tell how
+    many such keys it has.  n terms of one sign pattern are summed in fp32: n 2^-24 of the mean of |V|, in `check` 2^-14 of
+    it and 2^-11, of which V, normal and of 8 bits, leaves all but what 4500 terms need (2^-11.8)."""
+    from sageattention import sageattn
+
+    int8(monkeypatch, -1 if path == "int8" else sk)
+    monkeypatch.setenv("SAGEATTN_KV_SPLITS", "1")
+    q, k, v, top = make(sq, sk, d, BF16, a, b, 0.975 if a * b > 0 else 1.025 if b > LOWEST else None)
+    if causal:
+        top[:] = True
+        k[..., 0] = b
+    o, lse = sageattn(q, k, v, is_causal=causal, return_lse=True)
+    w = top.expand(sq, sk).float()
+    check(o, lse, q, k, v, w.tril() if causal else w, path)

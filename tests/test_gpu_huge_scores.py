@@ -164,8 +164,8 @@ def test_scores_on_both_sides_of_the_line(sign, order, path, sq, d, monkeypatch)
 @pytest.mark.parametrize("sq,sk,causal", [(200, 2300, False), (300, 4500, False), (2300, 2300, True), (130, 1100, False)])
 def test_equal_scores_of_many_keys(a, b, d, path, sq, sk, causal, monkeypatch):
     """Many key tiles of a wave (the pipelined steps), two key groups of a block.  Unsplit: a split's LSE does not tell how
-    many such keys it has.  n terms of one sign pattern are summed in fp32: n 2^-24 of the mean of |V|, in `check` 2^-14 of
-    it and 2^-11, of which V, normal and of 8 bits, leaves all but what 4500 terms need (2^-11.8)."""
+    many such keys it has.  bf16 V is exact in fp16, so the 2^-11 that `check` allows for it is there for the sums: 4500
+    terms, 2^-11.8 of the mean of |V| at most."""
     from sageattention import sageattn
 
     int8(monkeypatch, -1 if path == "int8" else sk)

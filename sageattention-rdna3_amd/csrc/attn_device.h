@@ -115,7 +115,7 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 // below it, in the product and in the row's max (huge_scale).  Differences of
 // scores are then down to half as large, but they are those of fp32 sums whose
 // steps are 1 or more; the LSE takes the max back to the scale (unscaled_max).
-// Otherwise: the score is rounded before the max is subtracted (huge_score).
+// Otherwise: the score is rounded before the max is subtracted.
 __device__ __forceinline__ bool huge_ref(float m) {
   // 2^24 <= |m| < FLT_MAX, in integers (their literals need no scalar registers, which the attention kernels spill)
   return (__float_as_uint(m) & 0x7fffffffu) - 0x4b800000u < 0x7f7fffffu - 0x4b800000u;
@@ -126,11 +126,6 @@ __device__ __forceinline__ float huge_scale(float sc) {
 // rsc: the row's scale, sc or huge_scale(sc)
 __device__ __forceinline__ float unscaled_max(float m, float rsc, float sc) {
   return rsc == sc ? m : m * __builtin_amdgcn_rcpf(rsc) * sc;
-}
-__device__ __forceinline__ float huge_score(float x, float sc, float m) {
-#pragma clang fp contract(off)
-  const float s = x * sc;
-  return huge_ref(m) ? s - m : __builtin_fmaf(x, sc, -m);
 }
 
 // Uniform 64-bit pointer (the compiler cannot always prove it).

@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_attn_kernel(FewParams p) {
     half8_t pf[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float sc[2] = {qs[rt] * ks[0], qs[rt] * ks[1]};
+      float sc[2] = {qs[rt] * ks[0], qs[rt] * ks[1]};
       float y[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) y[r] = static_cast<float>(s[rt][r]);
@@ -389,16 +389,17 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_attn_kernel(FewParams p) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[rt][db][r] *= alpha;
         }
+        if (huge[rt]) {  // such rows round the score here, like the max
+          const bool h = huge_ref(m_new);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[r] = h ? y[r] * sc[r >> 3] : y[r];
+          sc[0] = h ? 1.0f : sc[0];
+          sc[1] = h ? 1.0f : sc[1];
+        }
       }
       // score - max in one rounding: scores may be far larger than their differences
-      if (huge[rt]) {
-        asm volatile("");  // a real branch
 #pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] = huge_score(y[r], sc[r >> 3], m_run[rt]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc[r >> 3], -m_run[rt]);
-      }
+      for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc[r >> 3], -m_run[rt]);
       mask();
       float sum[2] = {0.0f, 0.0f};
       uint32_t pw[8];
